@@ -25,6 +25,7 @@ extern "C" {
 
 #define NVHIP_DTYPE_F32 0
 #define NVHIP_DTYPE_BF16 1
+#define NVHIP_DTYPE_F16 2
 
 #define NVHIP_PREC_IEEE 0 /* fp32 inputs used as they are */
 #define NVHIP_PREC_TF32 1 /* fp32 inputs rounded to a 10-bit mantissa (tf32) before the products */
@@ -284,6 +285,62 @@ int nvhip_qk_norm_rope_kv_decode_attention_bf16(
 int64_t nvhip_argmax_workspace_size(int64_t rows, int64_t n);
 int nvhip_argmax_bf16(int64_t* out, const void* logits, int64_t rows, int64_t n, int64_t row_stride,
                       void* workspace, int64_t workspace_size, void* stream);
+
+/*
+ * The 8-bit KV cache (the MX format of the OCP specification with e4m3 elements): codes [num_blocks, Hkv, block_size, D]
+ * and scales [num_blocks, Hkv, block_size, D / 32], a byte each. 32 consecutive elements of a head row share a scale byte
+ * e + 127; an element is code * 2^e. Storing divides a block by the least power of two (2^-117 at least) that brings its
+ * largest finite magnitude to 448 or below and rounds to the nearest code, ties to even; an infinity or a NaN becomes the
+ * NaN code. Every value is exact in bf16. Not in the reference: an 8-bit counterpart of its paged cache
+ * (model_runner.py:262-267) and of store_kvcache (layers/attention.py:34-41).
+ */
+
+/*
+ * Quantises token t's rows of key and value (row t at + t * {key,value}_stride elements, heads and elements contiguous;
+ * dtype NVHIP_DTYPE_BF16, F16 or F32) into slot slot_mapping[t] (page slot / block_size) of the caches. Slots outside
+ * [0, num_blocks * block_size) -- the padding value -1 -- are skipped. Of two tokens with the same slot in one call either
+ * may win, element by element: give each slot once. D: 64, 128 or 256; caches and scales 16-byte aligned.
+ */
+int nvhip_store_kvcache_mxfp8(void* k_cache, void* v_cache, void* k_scales, void* v_scales, const void* key,
+                              const void* value, int64_t key_stride, int64_t value_stride, const int32_t* slot_mapping,
+                              int64_t num_blocks, int64_t block_size, int64_t n, int64_t Hkv, int64_t D, int dtype,
+                              void* stream);
+
+/*
+ * Reads sequences back: row cu_seqlens_k[b] + j of k and v ([total, Hkv, D] bf16, contiguous) is token j of the pages of
+ * block_table row b ([num_seqs, max_blocks]), for j < cu_seqlens_k[b + 1] - cu_seqlens_k[b]. Rows behind the last
+ * sequence and tokens without a valid page (an entry outside [0, num_blocks), or past max_blocks) are zeros. The layout is
+ * that of nvhip_prefill_attention_bf16 without a block table, so a prompt chunk over a cached prefix is this call and that.
+ */
+int nvhip_load_kvcache_mxfp8(void* k, void* v, const void* k_cache, const void* v_cache, const void* k_scales,
+                             const void* v_scales, const int32_t* block_table, const int32_t* cu_seqlens_k,
+                             int64_t num_seqs, int64_t total, int64_t Hkv, int64_t D, int64_t block_size,
+                             int64_t num_blocks, int64_t max_blocks, void* stream);
+
+/*
+ * Attention of q_len <= 64 query tokens per sequence over a paged cache: the tree of drafted tokens of a speculative
+ * step, and the decode step of the 8-bit cache.
+ *   q, out [num_seqs * q_len, Hq, D] bf16 (strides in elements; q 16-byte aligned rows, multiples of 8);
+ *   k_scales, v_scales null: bf16 caches [num_blocks, block_size, Hkv, D] (nvhip_paged_decode_attention_bf16's); given:
+ *   the 8-bit caches above. block_table [num_seqs, max_blocks] int32, context_lens [num_seqs] int32: the cached tokens of
+ *   each sequence, the q_len query tokens last. Query i sees every token before them and, of them, token j where bit j of
+ *   tree_mask[b * q_len + i] is set (tree_mask null: j <= i if causal, else all). With fewer than q_len cached tokens the
+ *   first of the query tokens are the ones that are missing. A query that sees nothing gets zeros; tokens in no valid
+ *   page take no part; what lies in tokens that a query does not see, NaN included, does not reach its row.
+ *   scale > 0. workspace (16-byte aligned, contents need no initialisation) of nvhip_tree_attention_workspace_size bytes
+ *   lets blocks share a context; with a NULL (or too small) workspace one block takes each (sequence, kv head, 16 rows).
+ *   Calls may run at the same time as long as each has its own workspace; the result does not depend on timing.
+ */
+int nvhip_tree_attention(void* out, const void* q, const void* k_cache, const void* v_cache, const void* k_scales,
+                         const void* v_scales, const int32_t* block_table, const int32_t* context_lens,
+                         const int64_t* tree_mask, int64_t num_seqs, int64_t q_len, int64_t Hq, int64_t Hkv, int64_t D,
+                         int64_t block_size, int64_t num_blocks, int64_t max_blocks, int64_t q_stride_token,
+                         int64_t q_stride_head, int64_t out_stride_token, int64_t out_stride_head, float scale,
+                         int causal, void* workspace, int64_t workspace_size, void* stream);
+
+/* Bytes of workspace nvhip_tree_attention can use for these sizes. Host-only, no GPU work. */
+int64_t nvhip_tree_attention_workspace_size(int64_t num_seqs, int64_t q_len, int64_t Hq, int64_t Hkv, int64_t D,
+                                            int64_t block_size, int64_t max_blocks);
 
 #ifdef __cplusplus
 }

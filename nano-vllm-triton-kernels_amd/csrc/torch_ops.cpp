@@ -14,6 +14,7 @@
 #include <torch/library.h>
 
 #include <algorithm>
+#include <initializer_list>
 #include <mutex>
 #include <optional>
 #include <string>
@@ -68,6 +69,12 @@ void* attention_workspace(const Tensor& q, int64_t nbytes) {
     held.push_back(at::zeros({std::max<int64_t>(nbytes, int64_t(1) << 20)}, q.options().dtype(at::kByte)));
   }
   return held.back().data_ptr();
+}
+
+// The tensors of a call have to be on one device: a kernel that reads another's memory faults.
+void same_device(const char* what, const Tensor& a, std::initializer_list<const Tensor*> others) {
+  for (const Tensor* t : others)
+    TORCH_CHECK_VALUE(t->device() == a.device(), what, ": tensors on ", a.device(), " and ", t->device());
 }
 
 std::tuple<Tensor, Tensor> qk_norm_rope_kv(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& positions,
@@ -262,6 +269,59 @@ Tensor argmax(const Tensor& logits) {
   return out;
 }
 
+void store_kvcache_mxfp8(const Tensor& key, const Tensor& value, const Tensor& k_cache, const Tensor& v_cache,
+                         const Tensor& k_scales, const Tensor& v_scales, const Tensor& slot_mapping) {
+  same_device("store_kvcache_mxfp8", key, {&value, &k_cache, &v_cache, &k_scales, &v_scales, &slot_mapping});
+  const c10::DeviceGuard guard(key.device());
+  const at::ScalarType type = key.scalar_type();
+  check(nvhip_store_kvcache_mxfp8(
+            k_cache.data_ptr(), v_cache.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(), key.data_ptr(),
+            value.data_ptr(), key.stride(0), value.stride(0), i32(slot_mapping), k_cache.size(0), k_cache.size(2),
+            key.size(0), key.size(1), key.size(2),
+            type == at::kBFloat16 ? NVHIP_DTYPE_BF16 : type == at::kHalf ? NVHIP_DTYPE_F16 : NVHIP_DTYPE_F32,
+            stream_of(key)),
+        "store_kvcache_mxfp8");
+}
+
+std::tuple<Tensor, Tensor> load_kvcache_mxfp8(const Tensor& k_cache, const Tensor& v_cache, const Tensor& k_scales,
+                                              const Tensor& v_scales, const Tensor& block_table, const Tensor& cu_k,
+                                              int64_t total) {
+  same_device("load_kvcache_mxfp8", k_cache, {&v_cache, &k_scales, &v_scales, &block_table, &cu_k});
+  const c10::DeviceGuard guard(k_cache.device());
+  const int64_t Hkv = k_cache.size(1), bs = k_cache.size(2), D = k_cache.size(3);
+  const auto opts = k_cache.options().dtype(at::kBFloat16);
+  Tensor k = at::empty({total, Hkv, D}, opts), v = at::empty({total, Hkv, D}, opts);
+  check(nvhip_load_kvcache_mxfp8(k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_scales.data_ptr(),
+                                 v_scales.data_ptr(), i32(block_table), i32(cu_k), cu_k.size(0) - 1, total, Hkv, D, bs,
+                                 k_cache.size(0), block_table.size(1), stream_of(k_cache)),
+        "load_kvcache_mxfp8");
+  return {k, v};
+}
+
+// q [num_seqs, q_len, Hq, D]. The workspace is the call's own: calls on several streams, and captured calls, which keep
+// theirs in the graph's memory, do not meet in it.
+Tensor tree_attention(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache, const std::optional<Tensor>& k_scales,
+                      const std::optional<Tensor>& v_scales, const Tensor& block_table, const Tensor& context_lens,
+                      const std::optional<Tensor>& mask, double scale, bool causal) {
+  same_device("tree_attention", q, {&k_cache, &v_cache, &block_table, &context_lens});
+  const bool mx = k_scales.has_value();
+  if (mx) same_device("tree_attention", q, {&*k_scales, &*v_scales});
+  if (mask.has_value()) same_device("tree_attention", q, {&*mask});
+  const c10::DeviceGuard guard(q.device());
+  const int64_t B = q.size(0), n = q.size(1), Hq = q.size(2), D = q.size(3), num_blocks = k_cache.size(0),
+                Hkv = k_cache.size(mx ? 1 : 2), bs = k_cache.size(mx ? 2 : 1), max_blocks = block_table.size(1);
+  Tensor out = at::empty({B, n, Hq, D}, q.options());
+  const int64_t need = nvhip_tree_attention_workspace_size(B, n, Hq, Hkv, D, bs, max_blocks);
+  Tensor ws = at::empty({need}, q.options().dtype(at::kByte));
+  check(nvhip_tree_attention(out.data_ptr(), q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+                             mx ? k_scales->data_ptr() : nullptr, mx ? v_scales->data_ptr() : nullptr, i32(block_table),
+                             i32(context_lens), mask.has_value() ? i64(*mask) : nullptr, B, n, Hq, Hkv, D, bs, num_blocks,
+                             max_blocks, q.stride(1), q.stride(2), out.stride(1), out.stride(2), float(scale),
+                             int(causal), need ? ws.data_ptr() : nullptr, need, stream_of(q)),
+        "tree_attention");
+  return out;
+}
+
 }  // namespace
 
 TORCH_LIBRARY_IMPL(nvhip, CUDA, m) {
@@ -280,4 +340,7 @@ TORCH_LIBRARY_IMPL(nvhip, CUDA, m) {
   m.impl("store_kvcache", store_kvcache);
   m.impl("paged_decode_attention", paged_decode_attention);
   m.impl("argmax", argmax);
+  m.impl("store_kvcache_mxfp8", store_kvcache_mxfp8);
+  m.impl("load_kvcache_mxfp8", load_kvcache_mxfp8);
+  m.impl("tree_attention", tree_attention);
 }

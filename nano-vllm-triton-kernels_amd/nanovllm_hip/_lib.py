@@ -11,13 +11,14 @@ import torch  # noqa: F401  (must be loaded before the HIP library, see above)
 
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libnvhip.so")
 TORCH_LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libnvhip_torch.so")  # the torch ops
-ABI_VERSION = 7
+ABI_VERSION = 8
 
 NVHIP_OK = 0
 NVHIP_EINVAL = -1
 NVHIP_ELAUNCH = -2
 DTYPE_F32 = 0
 DTYPE_BF16 = 1
+DTYPE_F16 = 2
 PREC_IEEE = 0
 PREC_TF32 = 1
 
@@ -54,10 +55,16 @@ SIGNATURES = {
                                                     _i64, _i64, _f, _p, _i64, _p],
     "nvhip_argmax_workspace_size": [_i64, _i64],
     "nvhip_argmax_bf16": [_p, _p, _i64, _i64, _i64, _p, _i64, _p],
+    "nvhip_store_kvcache_mxfp8": [_p, _p, _p, _p, _p, _p, _i64, _i64, _p, _i64, _i64, _i64, _i64, _i64, _i, _p],
+    "nvhip_load_kvcache_mxfp8": [_p, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _p],
+    "nvhip_tree_attention": [_p, _p, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
+                             _i64, _i64, _i64, _f, _i, _p, _i64, _p],
+    "nvhip_tree_attention_workspace_size": [_i64, _i64, _i64, _i64, _i64, _i64, _i64],
 }
 RESTYPES = {"nvhip_last_error": ctypes.c_char_p, "nvhip_paged_decode_attention_workspace_size": ctypes.c_int64,
             "nvhip_prefill_attention_workspace_size": ctypes.c_int64,
-            "nvhip_matmul_add_rms_norm_workspace_size": ctypes.c_int64, "nvhip_argmax_workspace_size": ctypes.c_int64}
+            "nvhip_matmul_add_rms_norm_workspace_size": ctypes.c_int64, "nvhip_argmax_workspace_size": ctypes.c_int64,
+            "nvhip_tree_attention_workspace_size": ctypes.c_int64}
 
 _lib = None
 

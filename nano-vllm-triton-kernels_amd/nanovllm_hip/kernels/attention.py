@@ -18,6 +18,7 @@ csrc/paged_attention.hip.
 import torch
 
 import nanovllm_hip.ops  # noqa: F401  (registers torch.ops.nvhip)
+from nanovllm_hip.kernels.kvcache_mxfp8 import check_caches
 
 
 def flash_attn_with_kvcache(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -124,3 +125,67 @@ def flash_attn_varlen_func(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, ma
         return out
     return torch.ops.nvhip.prefill_attention(q, k, v, cu_seqlens_q.contiguous(), cu_seqlens_k.contiguous(),
                                              int(max_seqlen_q), int(max_seqlen_k), scale, causal, block_table)
+
+
+def _few_queries(q, k_cache, v_cache, k_scales, v_scales, cache_seqlens, block_table, mask, softmax_scale, causal):
+    assert q.dim() == 4 and q.dtype == torch.bfloat16, (q.shape, q.dtype)
+    B, n, Hq, D = q.shape
+    assert 1 <= n <= 64, n
+    if k_scales is None:
+        assert k_cache.dim() == 4 and k_cache.shape == v_cache.shape, (k_cache.shape, v_cache.shape)
+        assert k_cache.dtype == v_cache.dtype == torch.bfloat16
+        assert k_cache.is_contiguous() and v_cache.is_contiguous()
+        Hkv = k_cache.shape[2]
+    else:
+        check_caches(k_cache, v_cache, k_scales, v_scales)
+        Hkv = k_cache.shape[1]
+    assert k_cache.shape[3] == D and D in (64, 128, 256), (k_cache.shape, D)
+    assert Hq % Hkv == 0, (Hq, Hkv)
+    assert block_table.dtype == torch.int32 and block_table.dim() == 2 and block_table.shape[0] == B
+    assert cache_seqlens.dtype == torch.int32 and cache_seqlens.shape == (B,)
+    st = q.stride()
+    if (st[3] != 1 or st[2] % 8 or st[1] % 8 or st[2] < D or st[1] < Hq * st[2] or (B > 1 and st[0] != n * st[1])
+            or q.data_ptr() % 16):
+        q = q.clone(memory_format=torch.contiguous_format)
+    scale = D ** -0.5 if softmax_scale is None else float(softmax_scale)
+    return torch.ops.nvhip.tree_attention(q, k_cache, v_cache, k_scales, v_scales, block_table.contiguous(),
+                                          cache_seqlens.contiguous(), mask, scale, causal)
+
+
+def flash_attn_with_kvcache_mxfp8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scales: torch.Tensor,
+                                  v_scales: torch.Tensor, cache_seqlens: torch.Tensor, block_table: torch.Tensor,
+                                  softmax_scale: float | None = None, causal: bool = False) -> torch.Tensor:
+    """flash_attn_with_kvcache over the 8-bit cache (layout and format: kernels.kvcache_mxfp8): q [num_seqs, q_len, Hq, D]
+    bf16, q_len <= 64 -> o, the same shape. The codes are read as what they stand for, exactly; the arithmetic is that of
+    the bf16 cache's attention. Query i sees the cache up to cache_seqlens - q_len + i with causal=True, all of it
+    without; a query that sees nothing gets zeros. Kernel: csrc/tree_attention.hip."""
+    return _few_queries(q, k_cache, v_cache, k_scales, v_scales, cache_seqlens, block_table, None, softmax_scale, causal)
+
+
+def tree_attention_with_kvcache(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                                cache_seqlens: torch.Tensor, block_table: torch.Tensor, tree_mask: torch.Tensor,
+                                softmax_scale: float | None = None, k_scales: torch.Tensor | None = None,
+                                v_scales: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of a tree of n <= 64 drafted tokens per sequence, the step that verifies them: q [num_seqs, n, Hq, D] bf16
+    -> o, the same shape. The nodes' keys and values are stored first, as the sequence's last n cached tokens
+    (cache_seqlens counts them). Node i sees the tokens before the tree and, of the tree, node j where bit j of
+    tree_mask[b, i] is set: its ancestors and itself (tree_mask() makes the row of a tree from its nodes' parents).
+    tree_mask [num_seqs, n] int64; bits from n on are ignored. A node that sees nothing gets zeros; a batch of smaller trees
+    is padded with nodes that no mask names.
+    k_cache, v_cache: bf16 [num_blocks, block_size, Hkv, D], or, with k_scales and v_scales, the 8-bit caches of
+    kernels.kvcache_mxfp8. Kernel: csrc/tree_attention.hip."""
+    assert (k_scales is None) == (v_scales is None), "k_scales and v_scales are given together"
+    assert tree_mask.dtype == torch.int64 and tree_mask.shape == q.shape[:2], (tree_mask.dtype, tree_mask.shape)
+    return _few_queries(q, k_cache, v_cache, k_scales, v_scales, cache_seqlens, block_table, tree_mask.contiguous(),
+                        softmax_scale, False)
+
+
+def tree_mask(parents: list[int]) -> list[int]:
+    """The masks of a tree's nodes, as tree_attention_with_kvcache takes them, from each node's parent (an earlier node, or
+    -1 for a child of the last accepted token): bit j of entry i says that node i sees node j."""
+    assert len(parents) <= 64, len(parents)
+    masks = []
+    for i, p in enumerate(parents):
+        assert -1 <= p < i, f"node {i}: parent {p} is no earlier node"
+        masks.append((masks[p] if p >= 0 else 0) | 1 << i)
+    return [m - (1 << 64) if m >> 63 else m for m in masks]  # as int64

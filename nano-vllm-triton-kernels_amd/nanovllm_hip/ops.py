@@ -42,10 +42,17 @@ _DEF.define("store_kvcache(Tensor key, Tensor value, Tensor(a!) k_cache, Tensor(
 _DEF.define("paged_decode_attention(Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_table, "
             "Tensor context_lens, int q_len, float scale, bool causal) -> Tensor")
 _DEF.define("argmax(Tensor logits) -> Tensor")
+_DEF.define("store_kvcache_mxfp8(Tensor key, Tensor value, Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor(c!) k_scales, "
+            "Tensor(d!) v_scales, Tensor slot_mapping) -> ()")
+_DEF.define("load_kvcache_mxfp8(Tensor k_cache, Tensor v_cache, Tensor k_scales, Tensor v_scales, Tensor block_table, "
+            "Tensor cu_seqlens_k, int total_k) -> (Tensor, Tensor)")
+_DEF.define("tree_attention(Tensor q, Tensor k_cache, Tensor v_cache, Tensor? k_scales, Tensor? v_scales, "
+            "Tensor block_table, Tensor cache_seqlens, Tensor? tree_mask, float scale, bool causal) -> Tensor")
 
 _OPS = ("qk_norm_rope_kv", "rms_norm", "fused_add_rms_norm", "fused_add_rms_norm_", "silu_and_mul", "matmul",
         "matmul_silu_mul", "rms_norm_matmul", "matmul_add_rms_norm", "qk_norm_rope_kv_decode_attention",
-        "prefill_attention", "prefill_attention_out", "store_kvcache", "paged_decode_attention", "argmax")
+        "prefill_attention", "prefill_attention_out", "store_kvcache", "paged_decode_attention", "argmax", "store_kvcache_mxfp8",
+        "load_kvcache_mxfp8", "tree_attention")
 
 
 def _load():
@@ -170,3 +177,24 @@ def _prefill_attention_fake(q, k, v, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, m
 @torch.library.register_fake("nvhip::argmax")
 def _argmax_fake(logits):
     return torch.empty(logits.shape[0], dtype=torch.int64, device=logits.device)
+
+
+# ------------------------------------------------------------------ 8-bit KV cache: write, read back
+
+@torch.library.register_fake("nvhip::store_kvcache_mxfp8")
+def _store_kvcache_mxfp8_fake(key, value, k_cache, v_cache, k_scales, v_scales, slot_mapping):
+    return None
+
+
+@torch.library.register_fake("nvhip::load_kvcache_mxfp8")
+def _load_kvcache_mxfp8_fake(k_cache, v_cache, k_scales, v_scales, block_table, cu_seqlens_k, total_k):
+    shape = (total_k, k_cache.shape[1], k_cache.shape[3])
+    return (torch.empty(shape, dtype=torch.bfloat16, device=k_cache.device),
+            torch.empty(shape, dtype=torch.bfloat16, device=k_cache.device))
+
+
+# ------------------------------------------------------------------ a few query tokens over either cache
+
+@torch.library.register_fake("nvhip::tree_attention")
+def _tree_attention_fake(q, k_cache, v_cache, k_scales, v_scales, block_table, cache_seqlens, tree_mask, scale, causal):
+    return torch.empty(q.shape, dtype=q.dtype, device=q.device)
