@@ -222,6 +222,54 @@ def test_heads_dims_and_pages(cache, Hq, Hkv, D, bs):
 
 @gpu
 @pytest.mark.parametrize("cache", CACHES)
+@pytest.mark.parametrize("n,Hq,Hkv,D,bs", [(20, 4, 2, 64, 7), (33, 8, 4, 128, 40), (17, 8, 2, 256, 64), (9, 16, 4, 256, 24),
+                                            (64, 6, 2, 64, 64), (64, 2, 2, 128, 16), (11, 6, 1, 128, 192), (50, 3, 1, 256, 1)])
+def test_many_rows(cache, n, Hq, Hkv, D, bs):
+    """33 rows of a kv head and more, and row counts that leave waves without rows: pages that end inside a step of 64
+    tokens, missing pages, contexts shorter than the tree."""
+    c = Case([200, 64, 5, 1, 129], n, Hq, Hkv, D, bs, cache, seed=n + D)
+    if bs < 64:
+        c.table[0, 1] = -1
+    c.check(c())
+
+
+@gpu
+@pytest.mark.parametrize("cache", CACHES)
+def test_many_rows_over_long_contexts(cache):
+    c = Case([4000, 1, 700], 24, Hq=8, Hkv=2, D=64, bs=64, cache=cache, seed=21)
+    first = c()
+    c.check(first)
+    for _ in range(5):
+        assert torch.equal(c(), first)
+
+
+@gpu
+@pytest.mark.parametrize("bs", [16, 64])
+@pytest.mark.parametrize("what", [float("nan"), float("inf")])
+def test_many_rows_do_not_meet_what_they_do_not_see(bs, what):
+    for cache in CACHES:
+        c = Case([45, 130, 70], 40, Hq=4, Hkv=2, D=64, bs=bs, cache=cache, seed=22)
+        clean = c()
+        for bad in (3, 38):   # in the tree's first and last step of 64 tokens
+            t = 130 - 40 + bad
+            page, row = int(c.table[1, t // bs]), t % bs
+            if cache == "bf16":
+                c.caches[1][page, row] = what
+            else:
+                c.caches[1].view(torch.uint8)[page, :, row] = 0x7F
+        out = c()
+        assert torch.equal(out[0], clean[0]) and torch.equal(out[2], clean[2])
+        see = c.visible(1)[:, [130 - 40 + 3, 130 - 40 + 38]].any(1)
+        assert bool(see.any()) and not bool(see.all())
+        for i in range(40):
+            if not see[i]:
+                assert torch.equal(out[1, i], clean[1, i])
+            else:
+                assert bool((out[1, i] == what).all()) if cache == "bf16" and what == what else bool(out[1, i].isnan().all())
+
+
+@gpu
+@pytest.mark.parametrize("cache", CACHES)
 def test_long_contexts_are_shared_by_blocks(cache):
     c = Case([5000, 1, 3000], 9, Hq=4, Hkv=2, D=64, bs=32, cache=cache, seed=2)
     first = c()
