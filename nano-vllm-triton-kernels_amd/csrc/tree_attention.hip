@@ -87,6 +87,27 @@ struct Piece {
   int first, parts;          // blocks that share the unit: first .. first + parts - 1
 };
 
+// max / sum of v over lanes l and l ^ 16, in both lanes (v_permlane16_swap of v with itself: rows 0, 0, 2, 2 and 1, 1, 3, 3).
+__device__ __forceinline__ float pair16_max(float v) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float pair16_sum(float v) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// Inclusive scan of v over the wave by DPP: within rows of 16, then across them.
+template <class F>
+__device__ __forceinline__ int wave_scan(int v, F&& f) {
+  v = f(v, __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false));  // row_shr 1, 2, 4, 8
+  v = f(v, __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false));
+  v = f(v, __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false));
+  v = f(v, __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false));
+  v = f(v, __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false));  // row_bcast 15 into rows 1 and 3
+  return f(v, __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false));  // row_bcast 31 into rows 2 and 3
+}
+
 // 2^x by the hardware (within an ulp; below 2^-126 it is 0).
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
@@ -142,6 +163,10 @@ __device__ __forceinline__ void finish(const TreeArgs& g, const Piece& pc, int b
   constexpr int64_t kRecord = int64_t(RU) * (2 + D);
   // a block's record of the unit that it finishes, and of the one that it begins and does not finish
   float* rec = pc.parts > 1 ? g.ws + (2 * int64_t(block) + (block == pc.first ? 1 : 0)) * kRecord : nullptr;
+  // the unit's count, asked for early: what it says is only tried below, an old value does no harm
+  unsigned long long* word = g.counts + ((int64_t(pc.b) * g.Hkv + pc.h) * g.tiles + pc.tile) * kCountStride;
+  unsigned long long old = 0;
+  if (pc.parts > 1 && threadIdx.x == 0) old = __hip_atomic_load(word, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   auto write = [&](int r, int d, float o0, float o1) {
     const int rr = r0 + r, i = rr / g.G;
     const int64_t at = (int64_t(pc.b) * g.n + i) * g.o_st + int64_t(pc.h * g.G + rr - i * g.G) * g.o_sh + d;
@@ -164,9 +189,7 @@ __device__ __forceinline__ void finish(const TreeArgs& g, const Piece& pc, int b
 #pragma unroll
       for (int t = 0; t < D / 16; ++t) *reinterpret_cast<f32x4_t*>(&red_o[wave][l16][16 * t + 4 * h4]) = acc[rt][t];
     }
-    float l = l_run[rt];
-    l += __shfl_xor(l, 16);
-    l = pair32_sum(l);
+    const float l = pair32_sum(pair16_sum(l_run[rt]));
     if (h4 == 0) red_m[wave][l16] = m_run[rt], red_l[wave][l16] = l;
     __syncthreads();
     for (int idx = threadIdx.x; idx < min(16, rows - 16 * rt) * (D / 2); idx += kWaves * 64) {
@@ -195,8 +218,6 @@ __device__ __forceinline__ void finish(const TreeArgs& g, const Piece& pc, int b
   __syncthreads();
   int* flag = reinterpret_cast<int*>(red_m);
   if (threadIdx.x == 0) {
-    unsigned long long* word = g.counts + ((int64_t(pc.b) * g.Hkv + pc.h) * g.tiles + pc.tile) * kCountStride;
-    unsigned long long old = __hip_atomic_load(word, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     // the first to find another number (a later one's exchange fails: the number is there) puts this call's in its place,
     // itself counted; everybody else adds one
     if ((old & ~0xffffull) == g.call ||
@@ -211,7 +232,20 @@ __device__ __forceinline__ void finish(const TreeArgs& g, const Piece& pc, int b
   }
   __syncthreads();
   if (!*flag) return;
-  // every part's (max, sum) of every row in one round of loads; from them each part's share of the row's O
+  // 4 pairs of elements a thread and 4 parts at a time, 16 loads on the way, the first of them with the parts' (max, sum)
+  const int pairs = rows * (D / 2);
+  f32x2 o[4][4];
+  auto load_parts = [&](int i0, int k0) {
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+      for (int y = 0; y < 4; ++y) {
+        const int idx = min(i0 + y * kWaves * 64, pairs - 1);
+        o[u][y] = get(min(k0 + u, pc.parts - 1), 2 * RU + idx / (D / 2) * D + idx % (D / 2) * 2);
+      }
+  };
+  load_parts(threadIdx.x, 0);
+  // every part's (max, sum) of every row; from them each part's share of the row's O
   f32x2* ml = reinterpret_cast<f32x2*>(lds);  // [part][row]; the waves' O is no longer needed
   for (int i = threadIdx.x; i < pc.parts * rows; i += kWaves * 64) ml[i] = get(i / rows, 2 * (i % rows));
   __syncthreads();
@@ -227,19 +261,10 @@ __device__ __forceinline__ void finish(const TreeArgs& g, const Piece& pc, int b
     ml[r][1] = den;
   }
   __syncthreads();
-  // 4 pairs of elements a thread and 4 parts at a time: 16 loads on the way
-  const int pairs = rows * (D / 2);
   for (int i0 = threadIdx.x; i0 < pairs; i0 += 4 * kWaves * 64) {
     f32x2 sum[4] = {};
     for (int k0 = 0; k0 < pc.parts; k0 += 4) {
-      f32x2 o[4][4];
-#pragma unroll
-      for (int u = 0; u < 4; ++u)
-#pragma unroll
-        for (int y = 0; y < 4; ++y) {
-          const int idx = min(i0 + y * kWaves * 64, pairs - 1);
-          o[u][y] = get(min(k0 + u, pc.parts - 1), 2 * RU + idx / (D / 2) * D + idx % (D / 2) * 2);
-        }
+      if (k0 != 0 || i0 != int(threadIdx.x)) load_parts(i0, k0);
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
         if (k0 + u >= pc.parts) break;
@@ -313,8 +338,7 @@ __device__ __forceinline__ void softmax(const float* s, float scale_log2, float&
   float top = -INFINITY;
 #pragma unroll
   for (int e = 0; e < N; ++e) top = fmaxf(top, s[e]);
-  top = fmaxf(top, __shfl_xor(top, 16));  // the row's four lanes
-  top = pair32_max(top) * scale_log2;     // the scale is positive
+  top = pair32_max(pair16_max(top)) * scale_log2;  // over the row's four lanes; the scale is positive
   const bool move = top > m_run + 8.0f;   // also true for the first finite maximum (m_run = -inf)
   if (__ballot(move) != 0) {
     const float alpha = move ? exp2_fast(m_run - top) : 1.0f;  // 0 from m_run = -inf
@@ -387,8 +411,7 @@ __device__ __forceinline__ void add_token(const TreeArgs& g, int64_t r, int k, c
 #pragma unroll
         for (int i = 0; i < 4; ++i) s = __builtin_fmaf(float(qf[rt][x][e + i]), kk[i], s);
       }
-    s += __shfl_xor(s, 16);
-    s = pair32_sum(s) * g.scale_log2;
+    s = pair32_sum(pair16_sum(s)) * g.scale_log2;
     const bool yes = (see[rt] >> k) & 1;
     const float p = exp2_fast(s - (m_run[rt] == -INFINITY ? 0.0f : m_run[rt]));
 #pragma unroll
@@ -416,15 +439,15 @@ __device__ __forceinline__ void run_piece(const TreeArgs& g, const Piece& pc, in
   const int32_t* bt_row = g.bt + int64_t(b) * g.max_blocks;
   const int ch0 = pc.ch0 + wave, ch_end = min(pc.ch1, (ctx + kChunk - 1) / kChunk);
 
-  // The page of a chunk's first token (aligned) or of token lane % 32, one chunk ahead of its rows' loads.
-  auto load_page = [&](int ch) -> int {
-    if constexpr (ALIGNED) {
-      return load_uniform(bt_row + min(ch * kChunk, ctx - 1) / g.bs);
-    } else {
-      return bt_row[min(ch * kChunk + lane % 32, ctx - 1) / g.bs];
-    }
+  // The table's entry for the wave's next chunk, asked for one chunk ahead of its rows: aligned, of its page `at` (and `off`,
+  // where in the page it begins); else of token lane % 32.
+  const int last_page = (max(ctx, 1) - 1) / g.bs;
+  int at = ch0 * kChunk / g.bs, off = ch0 * kChunk - at * g.bs, page = 0;
+  auto ask_page = [&](int ch) {
+    if constexpr (ALIGNED) page = load_uniform(bt_row + min(at, last_page));
+    else page = bt_row[min(ch * kChunk + lane % 32, ctx - 1) / g.bs];
   };
-  int page = ch0 < ch_end ? load_page(ch0) : 0;
+  if (ch0 < ch_end) ask_page(ch0);
 
   // this lane's query rows, their dims in the order of the K operand's steps, and which of the last n tokens they see
   bf16x8_t qf[RT][KC];
@@ -472,7 +495,6 @@ __device__ __forceinline__ void run_piece(const TreeArgs& g, const Piece& pc, in
     const int t0 = ch * kChunk;
     int blk = page;
     if constexpr (ALIGNED) {  // a chunk lies in one page, whose rows behind the context may be read: one base, small offsets
-      const int off = t0 % g.bs;
       c.valid = ctx - t0 >= kChunk ? ~0u : (1u << (ctx - t0)) - 1;
       if (blk < 0 || blk >= g.num_blocks) blk = 0, c.valid = 0;
       const int64_t base = MX ? (int64_t(blk) * g.Hkv + h) * g.bs + off : (int64_t(blk) * g.bs + off) * g.Hkv + h;
@@ -497,11 +519,12 @@ __device__ __forceinline__ void run_piece(const TreeArgs& g, const Piece& pc, in
         for (int it = 0; it < PVI; ++it) c.vscale[it] = vsb[uint32_t((it * TPI + vt) * SB + vd / 2)];
       }
     } else {
-      const int t = t0 + lane % 32, off = min(t, ctx - 1) % g.bs;
+      const int t = t0 + lane % 32, in_page = min(t, ctx - 1) % g.bs;
       if (t >= ctx) blk = -1;
       c.valid = uint32_t(__ballot(blk >= 0 && blk < g.num_blocks));
       if (blk < 0 || blk >= g.num_blocks) blk = 0;
-      const int64_t base = MX ? (int64_t(blk) * g.Hkv + h) * g.bs + off : (int64_t(blk) * g.bs + off) * g.Hkv + h;
+      const int64_t base = MX ? (int64_t(blk) * g.Hkv + h) * g.bs + in_page
+                              : (int64_t(blk) * g.bs + in_page) * g.Hkv + h;
       auto row_of = [&](int j) -> int64_t {  // cache row of token t0 + j
         const uint32_t lo = __shfl(uint32_t(base), j), hi = __shfl(uint32_t(base >> 32), j);
         return int64_t((uint64_t(hi) << 32) | lo);
@@ -520,7 +543,9 @@ __device__ __forceinline__ void run_piece(const TreeArgs& g, const Piece& pc, in
         if constexpr (MX) c.vscale[it] = g.vs[r * SB + vd / 2];
       }
     }
-    page = load_page(ch + kWaves);
+    if constexpr (ALIGNED)
+      for (off += kWaves * kChunk; off >= g.bs; off -= g.bs) ++at;
+    ask_page(ch + kWaves);
   };
 
   uint64_t odd = 0;  // query tokens of this wave's chunks with a value that is not finite
@@ -657,11 +682,13 @@ __device__ __forceinline__ void run_wide(const TreeArgs& g, const Piece& pc, int
   uint32_t mine = 0;   // unaligned: bit p, this thread's row of pass p does
   uint64_t odd = 0;    // query tokens among this thread's rows with a value that is not finite
   const int ch_end = min(pc.ch1, (ctx + kStep - 1) / kStep);
-  // the pages of a step, one step ahead of its rows' loads
-  int page[ALIGNED ? 1 : NP];
-  auto load_pages = [&](int ch) {
+  // the table's entries for the next step, asked for one step ahead of its rows (aligned: its page `at`, which it begins
+  // `off` tokens into)
+  const int last_page = (max(ctx, 1) - 1) / g.bs;
+  int page[ALIGNED ? 1 : NP], at = pc.ch0 * kStep / g.bs, off = pc.ch0 * kStep - at * g.bs;
+  auto ask_pages = [&](int ch) {
     if constexpr (ALIGNED) {
-      page[0] = load_uniform(bt_row + min(ch * kStep, ctx - 1) / g.bs);
+      page[0] = load_uniform(bt_row + min(at, last_page));
     } else {
 #pragma unroll
       for (int p = 0; p < NP; ++p) page[p] = bt_row[min(ch * kStep + p * RPP + prow, ctx - 1) / g.bs];
@@ -671,7 +698,6 @@ __device__ __forceinline__ void run_wide(const TreeArgs& g, const Piece& pc, int
     const int t0 = ch * kStep;
     if constexpr (ALIGNED) {
       int blk = page[0];
-      const int off = t0 % g.bs;
       valid = ctx - t0 >= 64 ? ~0ull : (1ull << (ctx - t0)) - 1;
       if (blk < 0 || blk >= g.num_blocks) blk = 0, valid = 0;
       const int64_t base = MX ? (int64_t(blk) * g.Hkv + h) * g.bs + off
@@ -693,27 +719,28 @@ __device__ __forceinline__ void run_wide(const TreeArgs& g, const Piece& pc, int
       }
     } else {
       mine = 0;
-      int64_t at[NP];
+      int64_t rows[NP];
 #pragma unroll
       for (int p = 0; p < NP; ++p) {
-        const int t = t0 + p * RPP + prow, off = min(t, ctx - 1) % g.bs;
+        const int t = t0 + p * RPP + prow, in_page = min(t, ctx - 1) % g.bs;
         int blk = t < ctx ? page[p] : -1;
         if (blk < 0 || blk >= g.num_blocks) blk = 0;
         else mine |= 1u << p;
-        at[p] = MX ? (int64_t(blk) * g.Hkv + h) * g.bs + off
-                   : (int64_t(blk) * g.bs + off) * g.Hkv + h;
+        rows[p] = MX ? (int64_t(blk) * g.Hkv + h) * g.bs + in_page : (int64_t(blk) * g.bs + in_page) * g.Hkv + h;
       }
 #pragma unroll
       for (int p = 0; p < NP; ++p) {
-        kraw[p] = load16(g.kc + at[p] * RB, 16 * piece);
-        vraw[p] = load16(g.vc + at[p] * RB, 16 * piece);
+        kraw[p] = load16(g.kc + rows[p] * RB, 16 * piece);
+        vraw[p] = load16(g.vc + rows[p] * RB, 16 * piece);
         if constexpr (MX) {
-          kscale[p] = g.ks[at[p] * SB + piece / 2];
-          vscale[p] = g.vs[at[p] * SB + piece / 2];
+          kscale[p] = g.ks[rows[p] * SB + piece / 2];
+          vscale[p] = g.vs[rows[p] * SB + piece / 2];
         }
       }
     }
-    load_pages(ch + 1);
+    if constexpr (ALIGNED)
+      if ((off += kStep) == g.bs) off = 0, ++at;
+    ask_pages(ch + 1);
   };
   // The loaded rows into LDS. Of tokens that take no part, and of query tokens with a value that is not finite, the value is
   // zeros there: some rows may not see them, and 0 times them would be NaN.
@@ -784,7 +811,7 @@ __device__ __forceinline__ void run_wide(const TreeArgs& g, const Piece& pc, int
              [&](int t, const u32x4* f) { multiply(acc, t, f, phi + y, plo + y); });
   };
   if (pc.ch0 < ch_end) {
-    load_pages(pc.ch0);
+    ask_pages(pc.ch0);
     load_step(pc.ch0);
   }
   for (int ch = pc.ch0; ch < ch_end; ++ch) {
@@ -815,8 +842,7 @@ __device__ __forceinline__ void run_wide(const TreeArgs& g, const Piece& pc, int
   // another launch): (max, sum) of each row, then O [row][D]
   if (g.ws != nullptr && tid == 0 && block == pc.first)
     g.plan[(b * g.Hkv + h) * g.tiles + pc.tile] = int2{pc.first, pc.parts};
-  float l = l_run + __shfl_xor(l_run, 16);
-  l = pair32_sum(l);
+  const float l = pair32_sum(pair16_sum(l_run));
   if (row >= R) return;
   if (pc.parts == 1) {
     uint16_t* out = g.out + (int64_t(b) * g.n + qi) * g.o_st + int64_t(h * g.G + row - qi * g.G) * g.o_sh + 4 * h4;
@@ -868,15 +894,9 @@ __global__ __launch_bounds__(kWaves * 64, S::waves_per_simd(D)) void tree_attent
       const int w = S::start + chunks_of(min(max(g.ctx_lens[j], 0), g.max_blocks * g.bs));
       sum += w, longest = max(longest, w);
     }
-    int incl = sum;  // inclusive scan over the lanes
-#pragma unroll
-    for (int off = 1; off < 64; off *= 2) {
-      const int v = __shfl_up(incl, off);
-      if (lane >= off) incl += v;
-      longest = max(longest, __shfl_xor(longest, off));
-    }
+    const int incl = wave_scan(sum, [](int x, int y) { return x + y; });
     const int C = __builtin_amdgcn_readlane(incl, 63) * U;
-    longest = __builtin_amdgcn_readfirstlane(longest);
+    longest = __builtin_amdgcn_readlane(wave_scan(longest, [](int x, int y) { return max(x, y); }), 63);
     // A block takes enough that no unit lies in more than max_parts of them (one at either end), and, where the last of a
     // unit's blocks merges them alone, about the square root of (chunks x merging a part / a chunk): c chunks in P parts
     // take c / P of 0.4 us and P of 0.27 us (32 rows of 64; less with fewer rows).
