@@ -289,14 +289,15 @@ __device__ __forceinline__ void finish(const TreeArgs& g, const Piece& pc, int b
 // V^T fragments from LDS rows of pitch VP, two 16-dim tiles at a time, the next ones' reads issued before the products with
 // the ones at hand: f(tile, fragment). v: this lane's place in the first 4 x 16 block (row 4 (l / 16) + l % 16 / 4, dims
 // 4 (l % 4) ..): the transpose read hands the lanes of group l / 16 rows 4 (l / 16) .. + 3 (k slots 0..3), and 16 more (4..7).
-template <int DT, int VP>
+// TS: from a tile to the next in LDS.
+template <int DT, int VP, int TS = 16>
 struct VFragments {
   static constexpr int TP = 2;
   u32x4 f[2][TP];
   __device__ __forceinline__ void load(const uint16_t* v, int group) {
 #pragma unroll
     for (int i = 0; i < TP; ++i) {
-      const u32x2 lo = lds_read_tr16(v + 16 * (TP * group + i)), hi = lds_read_tr16(v + 16 * VP + 16 * (TP * group + i));
+      const u32x2 lo = lds_read_tr16(v + TS * (TP * group + i)), hi = lds_read_tr16(v + 16 * VP + TS * (TP * group + i));
       f[group % 2][i] = u32x4{lo[0], lo[1], hi[0], hi[1]};
     }
   }
@@ -641,10 +642,15 @@ __device__ __forceinline__ void run_piece(const TreeArgs& g, const Piece& pc, in
 // A unit of up to 64 rows: wave w has rows 16 w .. + 15, and a step is 64 tokens, which all waves bring into LDS in bf16
 // together (16 bytes of a row a lane, the next step's on the way meanwhile) and all read: what a step costs of the L2 and of
 // conversions is shared by all rows.
+// 8 bits: 16 codes become 32 bytes of bf16, and 8 lanes that wrote those one behind the other would meet on half of the
+// banks. The first 8 of each 16 elements lie in the first half of a row in LDS instead, the others in the second, so that 8
+// lanes write 128 bytes in a row; the rows of q are read in that order, and V's fragments from both halves (32 sequences of
+// 512 .. 2048 tokens with 128 rows: 73.0 -> 68.3 us).
 template <int D, bool MX, bool ALIGNED>
 __device__ __forceinline__ void run_wide(const TreeArgs& g, const Piece& pc, int block, unsigned char* lds) {
   constexpr int NU = kStep / 16;                // 16-token tiles of a step
-  constexpr int KP = D + 8, VP = D + 16;        // LDS row pitches: fragment reads on distinct banks
+  constexpr int KP = D + 8, VP = D + (MX ? 8 : 16);  // LDS row pitches: fragment reads on distinct banks
+  constexpr int HALF = MX ? D / 2 : 8;          // in LDS, from 8 elements to the next 8 of the row
   constexpr int KC = D / 32, DT = D / 16, EPL = MX ? 16 : 8, RB = MX ? D : 2 * D, SB = D / kMxBlock;
   constexpr int LPR = D / EPL, RPP = kWaves * 64 / LPR, NP = kStep / RPP;  // lanes per row, rows per pass, passes
   const int tid = threadIdx.x, lane = tid % 64, wave = __builtin_amdgcn_readfirstlane(tid / 64);
@@ -661,10 +667,12 @@ __device__ __forceinline__ void run_wide(const TreeArgs& g, const Piece& pc, int
 #pragma unroll
   for (int x = 0; x < KC; ++x) qf[0][x] = bf16x8_t{};
   uint64_t see[1] = {0};
+  // the dims of a K or q fragment: 8 elements at 32 x + 8 h4 of a row in LDS
+  auto dim = [&](int x) { return MX ? 16 * ((4 * x + h4) % LPR) + 8 * (4 * x / LPR) : 32 * x + 8 * h4; };
   if (row < R) {
-    const uint16_t* qp = g.q + (int64_t(b) * g.n + qi) * g.q_st + int64_t(h * g.G + row - qi * g.G) * g.q_sh + 8 * h4;
+    const uint16_t* qp = g.q + (int64_t(b) * g.n + qi) * g.q_st + int64_t(h * g.G + row - qi * g.G) * g.q_sh;
 #pragma unroll
-    for (int x = 0; x < KC; ++x) qf[0][x] = *reinterpret_cast<const bf16x8_t*>(qp + 32 * x);
+    for (int x = 0; x < KC; ++x) qf[0][x] = *reinterpret_cast<const bf16x8_t*>(qp + dim(x));
     see[0] = g.mask != nullptr ? uint64_t(g.mask[int64_t(b) * g.n + qi]) : g.causal ? (2ull << qi) - 1 : ~0ull;
   }
   const int before = ctx - g.n;
@@ -749,12 +757,12 @@ __device__ __forceinline__ void run_wide(const TreeArgs& g, const Piece& pc, int
 #pragma unroll
     for (int p = 0; p < NP; ++p) {
       const int j = p * RPP + prow;
-      uint16_t *kd = ks + j * KP + EPL * piece, *vd = vs + j * VP + EPL * piece;
+      uint16_t *kd = ks + j * KP + 8 * piece, *vd = vs + j * VP + 8 * piece;
       u32x4 v[MX ? 2 : 1];
       if constexpr (MX) {
         const float ka = mx_scale(kscale[p]), va = mx_scale(vscale[p]);
         *reinterpret_cast<u32x4*>(kd) = mx_decode8(kraw[p][0], kraw[p][1], ka);
-        *reinterpret_cast<u32x4*>(kd + 8) = mx_decode8(kraw[p][2], kraw[p][3], ka);
+        *reinterpret_cast<u32x4*>(kd + HALF) = mx_decode8(kraw[p][2], kraw[p][3], ka);
         v[0] = mx_decode8(vraw[p][0], vraw[p][1], va), v[1] = mx_decode8(vraw[p][2], vraw[p][3], va);
       } else {
         *reinterpret_cast<u32x4*>(kd) = kraw[p];
@@ -773,7 +781,7 @@ __device__ __forceinline__ void run_wide(const TreeArgs& g, const Piece& pc, int
           if (piece == 0) there[j] = in;
       }
 #pragma unroll
-      for (int x = 0; x < (MX ? 2 : 1); ++x) *reinterpret_cast<u32x4*>(vd + 8 * x) = v[x];
+      for (int x = 0; x < (MX ? 2 : 1); ++x) *reinterpret_cast<u32x4*>(vd + HALF * x) = v[x];
     }
   };
 
@@ -798,8 +806,8 @@ __device__ __forceinline__ void run_wide(const TreeArgs& g, const Piece& pc, int
 #pragma unroll
       for (int r = 0; r < 4; ++r) s[4 * u + r] = d[r];
     }
-    const uint16_t* v0 = vs + (4 * h4 + l16 / 4) * VP + 4 * (l16 % 4);
-    VFragments<DT, VP> vf;
+    const uint16_t* v0 = vs + (4 * h4 + l16 / 4) * VP + l16 % 4 / 2 * HALF + 4 * (l16 % 2);
+    VFragments<DT, VP, MX ? 8 : 16> vf;
     vf.load(v0, 0);
     __builtin_amdgcn_sched_barrier(0);
     if (masked) hide<4 * NU>(s, (visible(before - t0, see[0]) & live) >> (4 * h4));
@@ -835,7 +843,7 @@ __device__ __forceinline__ void run_wide(const TreeArgs& g, const Piece& pc, int
       const int k = __builtin_ctzll(odd), t = before + k, blk = bt_row[t / g.bs], off = t % g.bs;  // a valid page
       if (t / kStep < pc.ch0 || t / kStep >= pc.ch1) continue;
       add_token<D, MX, 1>(g, MX ? (int64_t(blk) * g.Hkv + h) * g.bs + off : (int64_t(blk) * g.bs + off) * g.Hkv + h, k, qf,
-                           see, m_run, acc, [&](int x) { return 32 * x + 8 * h4; });
+                           see, m_run, acc, dim);
     }
   }
   // to the output, or into a record that tree_combine_kernel merges with the other blocks' (through plain stores: that is
