@@ -320,7 +320,8 @@ int nvhip_load_kvcache_mxfp8(void* k, void* v, const void* k_cache, const void* 
 /*
  * Attention of q_len <= 64 query tokens per sequence over a paged cache: the tree of drafted tokens of a speculative
  * step, and the decode step of the 8-bit cache.
- *   q, out [num_seqs * q_len, Hq, D] bf16 (strides in elements; q 16-byte aligned rows, multiples of 8);
+ *   q, out [num_seqs * q_len, Hq, D] bf16 (strides in elements; q 16-byte aligned, strides multiples of 8; out 8-byte
+ *   aligned, strides multiples of 4); Hq <= 65536;
  *   k_scales, v_scales null: bf16 caches [num_blocks, block_size, Hkv, D] (nvhip_paged_decode_attention_bf16's); given:
  *   the 8-bit caches above. block_table [num_seqs, max_blocks] int32, context_lens [num_seqs] int32: the cached tokens of
  *   each sequence, the q_len query tokens last. Query i sees every token before them and, of them, token j where bit j of

@@ -28,7 +28,7 @@ __device__ __forceinline__ uint32_t mx_scale_byte(float a) {
   const uint32_t bits = __float_as_uint(fmaxf(a, 0x1p-109f));
   return (bits >> 23) - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);
 }
-// The byte as the float 2^e (e >= -126; the codes of a cache that was filled by other means may have a byte 0, read as 0).
+// The byte as the float 2^(byte - 127), of which 0 (no store writes it; the caches are zeros at first) reads as 0.
 __device__ __forceinline__ float mx_scale(uint32_t byte) { return __uint_as_float(byte << 23); }
 
 // |x| if x is finite, else 0.

@@ -305,6 +305,7 @@ Tensor tree_attention(const Tensor& q, const Tensor& k_cache, const Tensor& v_ca
                       const std::optional<Tensor>& mask, double scale, bool causal) {
   same_device("tree_attention", q, {&k_cache, &v_cache, &block_table, &context_lens});
   const bool mx = k_scales.has_value();
+  TORCH_CHECK_VALUE(mx == v_scales.has_value(), "tree_attention: k_scales and v_scales are given together");
   if (mx) same_device("tree_attention", q, {&*k_scales, &*v_scales});
   if (mask.has_value()) same_device("tree_attention", q, {&*mask});
   const c10::DeviceGuard guard(q.device());

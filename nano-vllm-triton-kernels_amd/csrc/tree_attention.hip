@@ -1048,7 +1048,8 @@ extern "C" int nvhip_tree_attention(void* out, const void* q, const void* k_cach
   if (!(scale > 0.0f) || scale > 3e38f) return invalid("tree_attention: softmax_scale must be positive and finite");
   if ((k_scales == nullptr) != (v_scales == nullptr))
     return invalid("tree_attention: k_scales and v_scales must be given together");
-  if (Hq > (1 << 20) || num_seqs > (1 << 24) || num_blocks > INT32_MAX || block_size > INT32_MAX ||
+  // (a head's rows of a page step lie up to 63 Hkv 2 D bytes apart, counted in 32 bits)
+  if (Hq > (1 << 16) || num_seqs > (1 << 24) || num_blocks > INT32_MAX || block_size > INT32_MAX ||
       max_blocks > INT32_MAX || max_blocks * block_size > INT32_MAX - 64)
     return invalid("tree_attention: size too large");
   if (num_seqs == 0) return NVHIP_OK;
@@ -1063,7 +1064,8 @@ extern "C" int nvhip_tree_attention(void* out, const void* q, const void* k_cach
   g.ks = static_cast<const uint8_t*>(k_scales), g.vs = static_cast<const uint8_t*>(v_scales);
   g.bt = block_table, g.ctx_lens = context_lens, g.mask = tree_mask;
   g.n = int(q_len), g.Hkv = int(Hkv), g.G = int(Hq / Hkv), g.bs = int(block_size), g.num_blocks = int(num_blocks);
-  g.max_blocks = int(max_blocks), g.num_seqs = int(num_seqs), g.tiles = int((R + rows - 1) / rows);
+  g.max_blocks = num_blocks > 0 ? int(max_blocks) : 0;  // without pages every context is empty
+  g.num_seqs = int(num_seqs), g.tiles = int((R + rows - 1) / rows);
   g.q_st = q_stride_token, g.q_sh = q_stride_head, g.o_st = out_stride_token, g.o_sh = out_stride_head;
   g.scale_log2 = scale * 1.4426950408889634f;
   g.causal = causal ? 1 : 0;

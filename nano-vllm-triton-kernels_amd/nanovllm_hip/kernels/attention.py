@@ -159,6 +159,7 @@ def flash_attn_with_kvcache_mxfp8(q: torch.Tensor, k_cache: torch.Tensor, v_cach
     bf16, q_len <= 64 -> o, the same shape. The codes are read as what they stand for, exactly; the arithmetic is that of
     the bf16 cache's attention. Query i sees the cache up to cache_seqlens - q_len + i with causal=True, all of it
     without; a query that sees nothing gets zeros. Kernel: csrc/tree_attention.hip."""
+    assert k_scales is not None and v_scales is not None, "the 8-bit cache has scales"
     return _few_queries(q, k_cache, v_cache, k_scales, v_scales, cache_seqlens, block_table, None, softmax_scale, causal)
 
 

@@ -115,6 +115,22 @@ def test_abi_refuses_without_launching():
     assert lib.nvhip_tree_attention_workspace_size(2, 3, 5, 2, 64, 16, 3) == 0
 
 
+def test_the_8_bit_cache_has_scales():
+    m = dict(device="meta")
+    q, lens = torch.empty(2, 1, 4, 64, dtype=BF16, **m), torch.empty(2, dtype=torch.int32, **m)
+    table, k = torch.empty(2, 3, dtype=torch.int32, **m), torch.empty(4, 16, 2, 64, dtype=BF16, **m)
+    with pytest.raises(AssertionError, match="scales"):
+        flash_attn_with_kvcache_mxfp8(q, k, k, None, None, lens, table)
+
+
+def test_abi_refuses_more_heads_than_offsets_count():
+    lib, A = _lib.lib(), ctypes.c_void_p(64)
+    Hq = (1 << 16) + 1
+    rc = lib.nvhip_tree_attention(A, A, A, A, None, None, A, A, None, 1, 1, Hq, Hq, 64, 64, 1, 1, Hq * 64, 64, Hq * 64, 64,
+                                  0.1, 0, None, 0, None)
+    assert rc == _lib.NVHIP_EINVAL and "too large" in lib.nvhip_last_error().decode()
+
+
 # ------------------------------------------------------------------ GPU
 
 class Case:
@@ -571,3 +587,23 @@ def test_tensors_on_two_devices_are_refused():
     with pytest.raises(ValueError, match="tensors on"):
         tree_attention_with_kvcache(c.q, *c.caches[:2], lens.to(DEV), table, c.mask, k_scales=c.caches[2],
                                     v_scales=c.caches[3])
+
+
+@gpu
+def test_one_scale_tensor_is_refused():
+    c = Case([40], 3, Hq=4, Hkv=2, D=64, bs=16)
+    lens, table = torch.tensor(c.lens, dtype=torch.int32, device=DEV), c.table.to(DEV)
+    for scales in ((c.caches[2], None), (None, c.caches[3])):
+        with pytest.raises(ValueError, match="together"):
+            torch.ops.nvhip.tree_attention(c.q, *c.caches[:2], *scales, table, lens, None, 0.1, False)
+
+
+@gpu
+@pytest.mark.parametrize("cache", CACHES)
+@pytest.mark.parametrize("n", [1, 20])
+def test_a_cache_without_pages(cache, n):
+    """No page is valid: no token takes part, whatever the table and the lengths say, and nothing is read."""
+    c = Case([40, 700], n, Hq=8, Hkv=2, D=64, bs=64, cache=cache, seed=13)
+    c.caches = [x[:0] for x in c.caches]
+    out = c()
+    assert out.shape == c.q.shape and bool((out == 0).all())
