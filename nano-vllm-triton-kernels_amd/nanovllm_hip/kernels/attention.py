@@ -137,8 +137,7 @@ def _few_queries(q, k_cache, v_cache, k_scales, v_scales, cache_seqlens, block_t
         assert k_cache.is_contiguous() and v_cache.is_contiguous()
         Hkv = k_cache.shape[2]
     else:
-        check_caches(k_cache, v_cache, k_scales, v_scales)
-        Hkv = k_cache.shape[1]
+        Hkv = check_caches(k_cache, v_cache, k_scales, v_scales)[1]
     assert k_cache.shape[3] == D and D in (64, 128, 256), (k_cache.shape, D)
     assert Hq % Hkv == 0, (Hq, Hkv)
     assert block_table.dtype == torch.int32 and block_table.dim() == 2 and block_table.shape[0] == B

@@ -32,7 +32,7 @@ def allocate_kvcache_mxfp8(num_blocks: int, block_size: int, num_kv_heads: int, 
 
 
 def check_caches(k_cache, v_cache, k_scales, v_scales):
-    """Asserts the layout above."""
+    """Asserts the layout above; the codes' shape."""
     shape = k_cache.shape
     assert len(shape) == 4 and shape == v_cache.shape and shape[3] in (64, 128, 256), (shape, v_cache.shape)
     assert k_cache.dtype == v_cache.dtype == torch.float8_e4m3fn, (k_cache.dtype, v_cache.dtype)
@@ -40,6 +40,7 @@ def check_caches(k_cache, v_cache, k_scales, v_scales):
     assert k_scales.shape == v_scales.shape == (shape[0], shape[1], shape[2], shape[3] // MX_BLOCK), k_scales.shape
     assert (k_cache.is_contiguous() and v_cache.is_contiguous() and k_scales.is_contiguous()
             and v_scales.is_contiguous())
+    return shape
 
 
 def store_kvcache_mxfp8(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -47,11 +48,12 @@ def store_kvcache_mxfp8(key: torch.Tensor, value: torch.Tensor, k_cache: torch.T
     """Quantises key, value [N, Hkv, D] (bf16, fp16 or fp32; heads contiguous, rows may be strided views of the qkv
     projection) into the slots slot_mapping [N] int32 (-1, or any slot outside the cache: skipped). A slot may be given
     once in a call: of two tokens in one slot, either may be what parts of the row hold."""
-    N, Hkv, D = key.shape
-    check_caches(k_cache, v_cache, k_scales, v_scales)
-    assert value.shape == key.shape and key.dtype == value.dtype and key.dtype in _TYPES, (key.dtype, value.dtype)
-    assert k_cache.shape[1] == Hkv and k_cache.shape[3] == D, (key.shape, k_cache.shape)
-    assert key.stride(2) == value.stride(2) == 1 and key.stride(1) == value.stride(1) == D
+    shape, dtype = key.shape, key.dtype
+    N, Hkv, D = shape
+    cache = check_caches(k_cache, v_cache, k_scales, v_scales)
+    assert value.shape == shape and value.dtype == dtype and dtype in _TYPES, (dtype, value.dtype)
+    assert cache[1] == Hkv and cache[3] == D, (shape, cache)
+    assert key.stride()[1:] == value.stride()[1:] == (D, 1), (key.stride(), value.stride())
     assert slot_mapping.dtype == torch.int32 and slot_mapping.shape == (N,)
     torch.ops.nvhip.store_kvcache_mxfp8(key, value, k_cache, v_cache, k_scales, v_scales, slot_mapping.contiguous())
 
