@@ -35,11 +35,14 @@
 //   512 units), which reads them with the whole card.
 // Calls may run at the same time on several streams as long as each has its own workspace.
 //
-// Times (8 kv heads of 128, G = 2, pages of 256, graph): 8-bit decode step of 1 sequence of 700 tokens 10.5 us (the chain of
-// loads: lengths, pages, rows, records), of 32 sequences of 512 .. 2048 24.9 us (3.8 TB/s), of 250 up to 4096 187-193 us
-// (5.4 TB/s; while streaming the blocks read at the card's rate, the rest is each piece's start and end); trees of 33 nodes
-// for 8 sequences of 1000 .. 4000, bf16, 37 us (2.2 TB/s); of 64 nodes for 32 sequences of 512 .. 2048, 8 bit, 72 us: there
-// the vector instructions of softmax and conversions (34 %), the matrix cores (23 %) and LDS (40 %) share the SIMDs' issue.
+// Times (8 kv heads of 128, G = 2, pages of 256; replayed from a graph). 8-bit decode step of 1 sequence of 700 tokens 10.5 us
+// (the chain of loads: lengths, pages, rows, records), of 32 sequences of 512 .. 2048 25 us (3.8 TB/s), of 250 up to 4096
+// 187 .. 193 us (5.4 TB/s; while streaming the blocks read at the card's rate, the rest is each piece's start and end). Trees
+// of 33 nodes for 8 sequences of 1000 .. 4000, bf16, 34.5 us (2.4 TB/s); of 64 nodes for 32 sequences of 512 .. 2048, 8 bit,
+// 67 us (0.35 PFLOP/s): products, softmax, staging, loads and the merge take what they take one after the other (leaving one
+// out saves 27, 11, 8, 8 and 10 us) although none fills its unit: vector issue 38 %, matrix cores 26 %, LDS 35 % of the
+// clocks. Two, three or four waves per SIMD, waves of 32 rows that read half as much of LDS, 128 rows to a block, and two LDS
+// buffers with one barrier a step took the same time within 3 %.
 #include <algorithm>
 #include <atomic>
 #include <random>

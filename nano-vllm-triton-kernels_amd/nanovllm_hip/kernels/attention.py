@@ -14,6 +14,9 @@ on the paged cache [num_blocks, block_size, Hkv, D] that the fused qk_norm_rope_
 below takes the same arguments and returns the same [num_seqs, q_len, Hq, D] output (query i of a sequence sees the
 cache up to context_len - q_len + i with causal=True; a sequence with context_len 0 gets zeros). The kernel is
 csrc/paged_attention.hip.
+
+Not in the reference, both csrc/tree_attention.hip: flash_attn_with_kvcache_mxfp8, the decode call over the 8-bit cache,
+and tree_attention_with_kvcache, the verification of a tree of drafted tokens over either cache.
 """
 import torch
 
