@@ -33,12 +33,13 @@
 //   upper 48 bits, and a word with another number counts as 0. It is left at 0 for the replays of a captured call.
 //   Of 64 rows a record is 33 KB, and one block took longer to merge them (up to 20 us) than a second launch does (10 us for
 //   512 units), which reads them with the whole card.
+// Short units are not split (Shape::whole).
 // Calls may run at the same time on several streams as long as each has its own workspace.
 //
 // Times (8 kv heads of 128, G = 2, pages of 256; replayed from a graph). 8-bit decode step of 1 sequence of 700 tokens 10.5 us
 // (the chain of loads: lengths, pages, rows, records), of 32 sequences of 512 .. 2048 25 us (3.8 TB/s), of 250 up to 4096
 // 187 .. 193 us (5.4 TB/s; while streaming the blocks read at the card's rate, the rest is each piece's start and end). Trees
-// of 33 nodes for 8 sequences of 1000 .. 4000, bf16, 34.5 us (2.4 TB/s); of 64 nodes for 32 sequences of 512 .. 2048, 8 bit,
+// of 33 nodes for 8 sequences of 1000 .. 4000, bf16, 33.0 us (2.5 TB/s); of 64 nodes for 32 sequences of 512 .. 2048, 8 bit,
 // 67 us (0.35 PFLOP/s): products, softmax, staging, loads and the merge take what they take one after the other (leaving one
 // out saves 27, 11, 8, 8 and 10 us) although none fills its unit: vector issue 38 %, matrix cores 26 %, LDS 35 % of the
 // clocks. Two, three or four waves per SIMD, waves of 32 rows that read half as much of LDS, 128 rows to a block, and two LDS
@@ -886,7 +887,11 @@ struct Shape {
   // What starting and finishing a piece costs beside its chunks, in chunks (measured per block: 4.4 us of 0.57 us a chunk, 10
   // of 0.6, and 4 us of 2 us): without it the blocks with many short units end last (250 sequences 218 -> 187 us).
   static constexpr int start = wide ? 2 : ROWS == 32 ? 16 : 8;
-  static constexpr int least = 8 * kChunk / tokens;             // chunks that a block takes at least
+  // Units of no more chunks than a start costs are not split: a second start and the merge took longer (484 units of 6 chunks
+  // 23.9 -> 20.0 us, 258 of 24 rows 22.3 -> 18.7; units of twice as many gain from the split: 208 of 10 .. 15 13.8 -> 13.2).
+  static constexpr int whole = 2 * start;
+  // chunks that a block takes at least (64 rows: a unit of one step; with 4, 5 sequences of up to 34 tokens 8.0 -> 11.5 us)
+  static constexpr int least = wide ? start + 1 : 8;
   static constexpr int max_parts = wide ? 64 : 2048 / rows;     // of a unit (not wide: their maxima and sums fit the LDS)
   static constexpr int waves_per_simd(int D) { return wide && D < 256 ? 3 : 2; }  // what the registers are laid out for
   static constexpr int blocks(int D) { return 256 * waves_per_simd(D); }          // of a split launch: all resident at once
@@ -941,9 +946,11 @@ __global__ __launch_bounds__(kWaves * 64, S::waves_per_simd(D)) void tree_attent
       ++b;
       continue;
     }
-    const int u = (at - begin) / w, u0 = begin + u * w + S::start, stop = min(end, u0 + c);  // u0: its first chunk
-    const int first = block_of(u0), last = block_of(u0 + c - 1);
-    if (stop > u0) {
+    const int u = (at - begin) / w, u0 = begin + u * w + S::start;  // u0: its first chunk
+    const bool whole = w <= S::whole, mine = !whole || at == u0 - S::start;  // a whole unit is of the block it begins in
+    const int stop = whole ? u0 + c : min(end, u0 + c);
+    const int first = whole ? p : block_of(u0), last = whole ? p : block_of(u0 + c - 1);
+    if (mine && stop > u0) {
       const Piece pc{b, u / g.tiles, u % g.tiles, max(at, u0) - u0, stop - u0, first, last - first + 1};
       if constexpr (S::wide) run_wide<D, MX, ALIGNED>(g, pc, p, lds);
       else run_piece<D, MX, ALIGNED, S::rows / 16>(g, pc, p, lds);
@@ -953,30 +960,70 @@ __global__ __launch_bounds__(kWaves * 64, S::waves_per_simd(D)) void tree_attent
   }
 }
 
-// The records of 64-row units that several blocks share, in the blocks' order: 4 elements a thread.
-template <int D>
-__global__ __launch_bounds__(256) void tree_combine_kernel(const TreeArgs g) {
-  constexpr int RU = 64, kSlices = RU * D / 1024;  // rows, blocks of a unit
-  const int unit = int(blockIdx.x) / kSlices, at = (int(blockIdx.x) % kSlices * 256 + int(threadIdx.x)) * 4;
+// The records of 64-row units that several blocks share: a lane has 4 elements of O. SPLIT waves share them, each with every
+// SPLIT-th record in the blocks' order, kAhead on the way at a time; their sums are joined in LDS.
+template <int D, int SPLIT>
+__global__ __launch_bounds__(kWaves * 64) void tree_combine_kernel(const TreeArgs g) {
+  constexpr int RU = 64, kSlices = RU * D * SPLIT / 1024, kAhead = SPLIT == 1 ? 4 : 8;  // rows, blocks of a unit
+  const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), k_first = wave % SPLIT;
+  const int unit = int(blockIdx.x) / kSlices;
+  const int at = ((int(blockIdx.x) % kSlices * kWaves + wave) / SPLIT * 64 + lane) * 4;
   const int2 plan = g.plan[unit];
   const int tile = unit % g.tiles, bh = unit / g.tiles, b = bh / g.Hkv, h = bh % g.Hkv;
   const int r = at / D, d = at % D, row = tile * RU + r;
-  if (plan.y == 1 || row >= g.G * g.n) return;
-  constexpr int64_t kRecord = int64_t(RU) * (2 + D);
-  auto record = [&](int k) { return g.ws + (2 * int64_t(plan.x + k) + (k == 0 ? 1 : 0)) * kRecord; };
+  if (plan.y == 1) return;
   float M = -INFINITY, den = 0.0f;
-#pragma unroll 4
-  for (int k = 0; k < plan.y; ++k) M = fmaxf(M, record(k)[2 * r]);
   f32x4_t sum = {0, 0, 0, 0};
-#pragma unroll 4
-  for (int k = 0; k < plan.y; ++k) {
-    const float* rec = record(k);
-    const float f = share(rec[2 * r], rec[2 * r + 1], M);
-    const f32x4_t o = *reinterpret_cast<const f32x4_t*>(rec + 2 * RU + r * D + d);
-    den = __builtin_fmaf(rec[2 * r + 1], f, den);
+  if (row < g.G * g.n) {
+    for (int k0 = k_first; k0 < plan.y; k0 += SPLIT * kAhead) {
+      f32x2 ml[kAhead];
+      f32x4_t o[kAhead];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) sum[e] = __builtin_fmaf(o[e], f, sum[e]);
+      for (int u = 0; u < kAhead; ++u) {
+        const int k = k0 + SPLIT * u;
+        ml[u] = f32x2{-INFINITY, 0.0f};
+        o[u] = f32x4_t{0, 0, 0, 0};
+        if (k >= plan.y) continue;
+        const float* rec = g.ws + (2 * int64_t(plan.x + k) + (k == 0 ? 1 : 0)) * (int64_t(RU) * (2 + D));
+        ml[u] = *reinterpret_cast<const f32x2*>(rec + 2 * r);
+        o[u] = *reinterpret_cast<const f32x4_t*>(rec + 2 * RU + r * D + d);
+      }
+      float top = M;
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) top = fmaxf(top, ml[u][0]);
+      const float keep = share(M, den, top);
+      M = top, den *= keep;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sum[e] *= keep;
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        const float f = share(ml[u][0], ml[u][1], M);
+        den = __builtin_fmaf(ml[u][1], f, den);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum[e] = __builtin_fmaf(o[u][e], f, sum[e]);
+      }
+    }
   }
+  if constexpr (SPLIT > 1) {
+    static_assert(SPLIT == kWaves, "the block's waves");
+    __shared__ float part[kWaves][6][64];
+    part[wave][0][lane] = M, part[wave][1][lane] = den;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) part[wave][2 + e][lane] = sum[e];
+    __syncthreads();
+    if (wave != 0) return;
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) M = fmaxf(M, part[w][0][lane]);
+    den = 0.0f, sum = f32x4_t{0, 0, 0, 0};
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      const float f = share(part[w][0][lane], part[w][1][lane], M);
+      den = __builtin_fmaf(part[w][1][lane], f, den);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sum[e] = __builtin_fmaf(part[w][2 + e][lane], f, sum[e]);
+    }
+  }
+  if (row >= g.G * g.n) return;
   const int i = row / g.G;
   uint16_t* out = g.out + (int64_t(b) * g.n + i) * g.o_st + int64_t(h * g.G + row - i * g.G) * g.o_sh + d;
   *reinterpret_cast<u32x2*>(out) = den == 0.0f ? u32x2{} : u32x2{pack_bf16x2(sum[0] / den, sum[1] / den),
@@ -990,13 +1037,17 @@ int launch(const TreeArgs& g, int64_t blocks, hipStream_t s) {
   else hipLaunchKernelGGL((tree_attention_kernel<D, MX, false, S>), grid, block, 0, s, g);
   if (int rc = check_launch("tree_attention")) return rc;
   if (!S::wide || g.ws == nullptr) return NVHIP_OK;
-  const int64_t slices = int64_t(g.num_seqs) * g.Hkv * g.tiles * (64 * D / 1024);
-  hipLaunchKernelGGL(tree_combine_kernel<D>, dim3(static_cast<unsigned>(slices)), dim3(256), 0, s, g);
+  // Few units: many records each, which the waves of a block share (8 units of up to 64 records 51.4 -> 45.0 us; 512 units
+  // of two or three 69.3 -> 73.2).
+  const int64_t units = int64_t(g.num_seqs) * g.Hkv * g.tiles, slices = units * (64 * D / 1024);
+  const dim3 one(static_cast<unsigned>(slices)), shared(static_cast<unsigned>(kWaves * slices));
+  if (units * 16 > blocks) hipLaunchKernelGGL((tree_combine_kernel<D, 1>), one, block, 0, s, g);
+  else hipLaunchKernelGGL((tree_combine_kernel<D, kWaves>), shared, block, 0, s, g);
   return check_launch("tree_attention (combine)");
 }
 
 // Rows of a unit for R = (Hq / Hkv) q_len rows of a kv head. 33 .. 64 rows as two units of 32 (8 sequences of 1000 .. 4000
-// tokens with 66 rows) took 53 us, as units of 64 rows 37.
+// tokens with 66 rows) took 53 us, as units of 64 rows 37 at that time.
 // Heads of 256 have no registers for two row tiles in a wave.
 int unit_rows(int64_t R, int64_t D) { return R <= 16 ? 16 : R <= 32 && D < 256 ? 32 : 64; }
 

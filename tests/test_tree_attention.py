@@ -251,6 +251,20 @@ def test_many_rows(cache, n, Hq, Hkv, D, bs):
 
 @gpu
 @pytest.mark.parametrize("cache", CACHES)
+@pytest.mark.parametrize("lens,n,Hq,Hkv", [
+    ([256, 257, 255, 288, 9] * 14, 1, 16, 8),            # 16 rows: contexts of 8 and 9 chunks of 32
+    ([512, 513, 511, 544, 30] * 10, 5, 16, 4),           # 32 rows: 16 and 17 chunks
+    ([128, 129, 127, 192, 40] * 8, 33, 4, 2),            # 64 rows: 2 and 3 steps of 64
+    ([900, 300, 700, 64, 1500, 10, 2000, 400], 33, 16, 8),   # 64 rows: two or three blocks to a unit
+])
+def test_short_units_and_shared_ones(cache, lens, n, Hq, Hkv):
+    """Units on both sides of the length from which they are split, more of them than a block takes."""
+    c = Case(lens, n, Hq=Hq, Hkv=Hkv, D=64, bs=64, cache=cache, seed=14)
+    c.check(c())
+
+
+@gpu
+@pytest.mark.parametrize("cache", CACHES)
 def test_many_rows_over_long_contexts(cache):
     c = Case([4000, 1, 700], 24, Hq=8, Hkv=2, D=64, bs=64, cache=cache, seed=21)
     first = c()
