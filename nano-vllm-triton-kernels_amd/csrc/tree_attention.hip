@@ -893,12 +893,15 @@ struct Shape {
   // chunks that a block takes at least (64 rows: a unit of one step; with 4, 5 sequences of up to 34 tokens 8.0 -> 11.5 us)
   static constexpr int least = wide ? start + 1 : 8;
   static constexpr int max_parts = wide ? 64 : 2048 / rows;     // of a unit (not wide: their maxima and sums fit the LDS)
-  static constexpr int waves_per_simd(int D) { return wide && D < 256 ? 3 : 2; }  // what the registers are laid out for
-  static constexpr int blocks(int D) { return 256 * waves_per_simd(D); }          // of a split launch: all resident at once
+  // What the registers are laid out for. bf16 rows of 256 elements: a chunk's rows and the sums take 390 registers; as two
+  // waves with 256 each, and the rest in scratch memory, 1 sequence of 11k tokens with 40 rows took 34.6 us for 20.8, 169 of 50
+  // with 4 rows 37.4 for 26.7.
+  static constexpr int waves_per_simd(int D, bool MX) { return D == 256 ? (MX ? 2 : 1) : wide ? 3 : 2; }
+  static constexpr int blocks(int D, bool MX) { return 256 * waves_per_simd(D, MX); }  // of a split launch: all resident at once
 };
 
 template <int D, bool MX, bool ALIGNED, class S>
-__global__ __launch_bounds__(kWaves * 64, S::waves_per_simd(D)) void tree_attention_kernel(const TreeArgs g) {
+__global__ __launch_bounds__(kWaves * 64, S::waves_per_simd(D, MX)) void tree_attention_kernel(const TreeArgs g) {
   __shared__ __attribute__((aligned(16))) unsigned char lds[lds_bytes(D, S::wide)];
   auto chunks_of = [](int ctx) { return max(1, (ctx + S::tokens - 1) / S::tokens); };
   const int U = g.Hkv * g.tiles;  // units of a sequence
@@ -1052,9 +1055,9 @@ int launch(const TreeArgs& g, int64_t blocks, hipStream_t s) {
 int unit_rows(int64_t R, int64_t D) { return R <= 16 ? 16 : R <= 32 && D < 256 ? 32 : 64; }
 
 // Blocks of the split launch: none without a chunk at the longest possible context.
-int64_t split_blocks(int64_t units, int64_t rows, int64_t D, int64_t max_ctx) {
+int64_t split_blocks(int64_t units, int64_t rows, int64_t D, bool mx, int64_t max_ctx) {
   const int64_t most = units * std::max<int64_t>(1, (max_ctx + kChunk - 1) / kChunk);
-  return std::min<int64_t>(rows == 64 ? Shape<64>::blocks(int(D)) : Shape<16>::blocks(int(D)), (most + 7) / 8 * 8);
+  return std::min<int64_t>(rows == 64 ? Shape<64>::blocks(int(D), mx) : Shape<16>::blocks(int(D), mx), (most + 7) / 8 * 8);
 }
 struct Workspace {
   int64_t count_bytes, bytes;
@@ -1083,7 +1086,8 @@ extern "C" int64_t nvhip_tree_attention_workspace_size(int64_t num_seqs, int64_t
   if (num_seqs <= 0 || q_len < 1 || Hq < 1 || Hkv < 1 || Hq % Hkv != 0 || D < 1 || block_size < 1 || max_blocks < 0)
     return 0;
   const int64_t R = Hq / Hkv * q_len, rows = unit_rows(R, D), units = num_seqs * Hkv * ((R + rows - 1) / rows);
-  return workspace_of(units, split_blocks(units, rows, D, max_blocks * block_size), rows, D).bytes;
+  // 8 bit: the launch with more blocks
+  return workspace_of(units, split_blocks(units, rows, D, true, max_blocks * block_size), rows, D).bytes;
 }
 
 extern "C" int nvhip_tree_attention(void* out, const void* q, const void* k_cache, const void* v_cache,
@@ -1137,7 +1141,7 @@ extern "C" int nvhip_tree_attention(void* out, const void* q, const void* k_cach
   if (units > INT32_MAX / 1024 || double(units) * double(max_blocks * block_size / kChunk + 2 + 64) > double(INT32_MAX))
     return invalid("tree_attention: size too large");
   int64_t blocks = units;
-  const int64_t split = split_blocks(units, rows, D, max_blocks * block_size);
+  const int64_t split = split_blocks(units, rows, D, k_scales != nullptr, max_blocks * block_size);
   const Workspace w = workspace_of(units, split, rows, D);
   if (workspace != nullptr && workspace_size >= w.bytes) {
     if (reinterpret_cast<uintptr_t>(workspace) % 16 != 0)
