@@ -31,7 +31,7 @@
 //   the XCDs' L2s are not coherent), waits for the stores and counts itself in; the one that completes the count reads the
 //   records back. The count is a word of the workspace that needs no initialisation: it holds a number of the call in its
 //   upper 48 bits, and a word with another number counts as 0. It is left at 0 for the replays of a captured call.
-//   Of 64 rows a record is 33 KB, and one block took longer to merge them (up to 20 us) than a second launch does (10 us for
+//   Of 64 rows a record is 33 KB, and one block took longer to merge them (up to 20 us) than a second launch does (9 us for
 //   512 units), which reads them with the whole card.
 // Short units are not split (Shape::whole).
 // Calls may run at the same time on several streams as long as each has its own workspace.
